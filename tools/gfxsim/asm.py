@@ -135,7 +135,7 @@ def parse_ins(text, lineno):
         return I
     rest = parts[1].strip()
     if I.base in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_waitcnt_vscnt", "s_waitcnt_depctr", "s_inst_prefetch", "s_clause", "s_setreg_imm32_b32",
-                  "s_setreg_b32", "s_getreg_b32", "s_sethalt", "s_trap", "s_icache_inv", "s_dcache_wb", "s_dcache_inv", "s_ttracedata", "s_sendmsg", "s_incperflevel",
+                  "s_setreg_b32", "s_getreg_b32", "s_sethalt", "s_trap", "s_icache_inv", "s_dcache_inv", "s_ttracedata", "s_sendmsg", "s_incperflevel",
                   "s_decperflevel"):
         I.aux = rest
         return I

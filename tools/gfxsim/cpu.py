@@ -566,7 +566,7 @@ def _branch_target(mod, I, pc):
 def _decode_salu(mod, I, pc):
     b, o = I.base, I.ops
     I.cls = "salu"
-    if b in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_waitcnt_vscnt", "s_waitcnt_depctr", "s_inst_prefetch", "s_clause", "s_icache_inv", "s_dcache_wb",
+    if b in ("s_waitcnt", "s_nop", "s_sleep", "s_setprio", "s_waitcnt_vscnt", "s_waitcnt_depctr", "s_inst_prefetch", "s_clause", "s_icache_inv",
              "s_dcache_inv", "s_setreg_imm32_b32", "s_setreg_b32", "s_ttracedata", "s_incperflevel", "s_decperflevel", "buffer_wbl2", "buffer_inv", "buffer_wbinvl1",
              "buffer_wbinvl1_vol", "s_sethalt"):
         I.cls = "other"
@@ -663,15 +663,6 @@ def _decode_salu(mod, I, pc):
                 if d in (126, 127):
                     raise SimError("s_load into exec")
                 w.S[d] = vals[j]
-        return f
-    if b.startswith("s_store_dword"):
-        I.cls = "smem"
-        n = {"": 1, "x2": 2, "x4": 4}[b.split("dword")[1]]
-        s0 = o[0][1]
-        gb, go = ssrc(o[1], 64), ssrc(o[2])
-        def f(w):
-            a = gb(w) + go(w)
-            w.mem.write_dwords(a, [w.S[s0 + j] for j in range(n)])
         return f
     # --- SOP1 / SOP2 / SOPC / SOPK -------------------------------------------------------------------------
     if b in ("s_mov_b32", "s_mov_b64", "s_cmov_b32", "s_cmov_b64"):
